@@ -4,7 +4,8 @@
 //
 // HBM bounds many rows: each logit is read once, 11.6 of them per cycle and SM in bf16 at the measured rate, next to 16 exponentials that the SM can
 // compute in it and about 128 instructions, of which one logit takes 6.5: pairs of fp32 go through one instruction where there is one (fma, add).  d is
-// one fma, so r may be rounded (the sums are in terms of r as it is).  Where |m| is beyond 2^96, as in rows of the type's lowest value, d is (x - m) log2 e.
+// one fma, so r may be rounded (the sums are in terms of r as it is): d of the maximum is then what the rounding left of it, at most 2^-4 up to |m| = 2^20.  It grows
+// with |m| and passes what 2^d can hold from 2^31 on, so beyond 2^20, as in rows masked throughout by a constant, d is (x - m) log2 e.
 // Every thread keeps its own sums over its share of the row, in terms of a reference that is renewed where an element is LP_AHEAD in front of it (with the
 // maximum itself one of 32 threads nearly always has to), and at the end in terms of the largest; they are joined then.  Batches come through a ring of
 // each thread's own in shared memory.
@@ -42,7 +43,7 @@ constexpr int LP_SHORT = 4096;   // elements of a row that one warp takes
 constexpr float LP_LN2 = 0.69314718055994531f, LP_LOG2E = 1.4426950408889634f;
 constexpr float LP_LOWEST = -3.402823466e38f;
 constexpr float LP_AHEAD = 5.f;                   // how far elements may be ahead of what the sums are in terms of; at the end that is the maximum
-constexpr float LP_FAR = 7.9228162514264338e28f;  // 2^96: maxima up to here, and elements from -2^100 on, have a log2 e multiple within fp32
+constexpr float LP_FAR = 1048576.f;               // 2^20: maxima up to here are within 2^-4 of their rounded multiple of log2 e
 
 using Key = unsigned long long;
 constexpr Key LP_FLOOR = (static_cast<Key>(0x007fffffu) << 32) | 0xffffffffu;  // above every element of -inf, below all others
@@ -191,14 +192,20 @@ template <int DT>
 __device__ __forceinline__ bool lp_far(float m) {
     return DT == WF_F16 ? m < -32768.f : fabsf(m) > LP_FAR;
 }
+// d of the maximum itself: what the rounding left of m log2 e, or nothing
+template <int DT>
+__device__ __forceinline__ float lp_rest(float m) {
+    return lp_far<DT>(m) ? 0.f : fmaf(m, LP_LOG2E, -__fmul_rn(m, LP_LOG2E));
+}
 
-// m, s and t of a part of a row, in terms of r = m log2 e as it is rounded
+// m, s and t of a part of a row, in terms of r = m log2 e as it is rounded (of m itself where that is far)
 struct LpSums {
     float m, s, t;
-    // the same sums in terms of a larger maximum
+    // the same sums in terms of a larger maximum.  (As the difference of the rounded multiples where neither is far: two branches more, up to 1% slower.)
     template <int DT>
     __device__ __forceinline__ void raise(float to) {
-        const float d = lp_far<DT>(m) || lp_far<DT>(to) ? (m - to) * LP_LOG2E : __fmul_rn(m, LP_LOG2E) - __fmul_rn(to, LP_LOG2E), f = lp_exp2(d), all = t + d * s;
+        const float d = fmaf(m - to, LP_LOG2E, lp_rest<DT>(to) - lp_rest<DT>(m));
+        const float f = lp_exp2(d), all = t + d * s;
         s *= f;
         t = f == 0.f ? s : f * all;  // 0, and d may be -inf; a NaN in s stays one
         m = to;
@@ -462,9 +469,9 @@ __global__ void __launch_bounds__(LP_THREADS, 7) logprobs_kernel(const LpParams 
     float row_m = 0.f, row_log = 0.f;
     auto finish = [&](const LpSums& a) {
         const bool empty = a.s == 0.f;  // every element is -inf
-        const float log2_s = log2f(a.s), rest = lp_far<DT>(a.m) ? 0.f : fmaf(a.m, LP_LOG2E, -__fmul_rn(a.m, LP_LOG2E));
+        const float log2_s = log2f(a.s);
         row_m = a.m;
-        row_log = LP_LN2 * (log2_s - rest);
+        row_log = LP_LN2 * (log2_s - lp_rest<DT>(a.m));
         if (lane == 0) {
             float lp = 0.f;
             if (tok >= p.V) lp = __uint_as_float(0x7fc00000u);
