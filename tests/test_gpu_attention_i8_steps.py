@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 def attention(q, cache, n, scale):
     """One sequence's n positions in float64, and what the kernel's arithmetic may be off by.  q [nq, d].  Half a step of a position's values is what 8 bits cannot tell
-    apart; what is asked for here is 2^-16 of that of the position that counts most, and rounding."""
+    apart; what is asked for here is 2^-27 of that of the position that counts most, for each position, and rounding."""
     nq, d = q.shape
     kc, vc, ks, vs = (c[0, :, :n].double() for c in cache)
     rep = nq // kc.shape[0]
@@ -24,8 +24,11 @@ def attention(q, cache, n, scale):
     w = p * vs
     out, size = torch.einsum("ht,htd->hd", w, vc), torch.einsum("ht,htd->hd", w, vc.abs())
     tol = torch.einsum("ht,htd->hd", w * off, vc.abs()) + out.abs() * (p * off).sum(-1, keepdim=True)
-    # p * step as two f16 numbers: 2^-21; what is below them: 2^-32 of the largest p * step for each position; fp32 sums in any order
-    tol += size * (2.0 ** -21 + 2.0 ** -23 * (n / 64 + 200)) + n * 2.0 ** -32 * 127 * w.amax(-1, keepdim=True)
+    # p * step as two f16 numbers: 2^-21; what is below them: the largest p * step is at least 2^3 of the range, f16 ends
+    # at 2^-24, so half of that is 2^-28 of the largest for each position; fp32 sums in any order
+    tol += size * (2.0 ** -21 + 2.0 ** -23 * (n / 64 + 200)) + n * 2.0 ** -28 * 127 * w.amax(-1, keepdim=True)
+    # fp32 powers of two end at 2^-126, taken relative to at most 2^9 times the largest: a weight below 2^-117 of that, give or take a score's error, may be 0
+    tol += (w * (p < 2.0 ** -116 * p.amax(-1, keepdim=True))).sum(-1, keepdim=True) * 127
     return out, tol
 
 

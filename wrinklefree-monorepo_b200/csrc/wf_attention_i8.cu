@@ -9,14 +9,18 @@
 // and the sums are exact.  An instruction has sixteen rows and a group of query heads at most eight: rows 0..7 hold the first digit and rows 8..15 the
 // second, a second instruction the third.
 // Values: p * v_step as a sum of two f16 numbers, 22 bits, in rows 0..7 and 8..15 of mma.sync.m16n8k16; the codes as f16, two at a time: byte ^ 0x80 in the
-// low bits of 1024.0, less 1152.  Range: p is taken relative to a maximum that is renewed only when a score is 2^8 ahead of it, v_step relative to the
-// power of two above the largest so far, times 2^7; the sum stays below 2^15 and resolves 2^-31.
+// low bits of 1024.0, less 1152.  Range: p is taken relative to 2^8 to 2^9 times its row's largest, and that is renewed when a score is ahead of it; p * v_step
+// relative to the row's largest so far, at 2^3 to 2^5 of the range, and renewed when one may be 2^10 ahead.  The sum stays below 2^15 and resolves 2^-28 of the
+// largest p * v_step of the row, of which half is what its position's codes cannot tell apart; p below 2^-117 of the largest is 0.  Whether to renew is asked of scores
+// and steps alone, before the exponents: a row's limit for scores allows for the largest step of the tile that renewed last.  (Relative to the largest step, whatever
+// its weight, other positions lost 0.4 % beside a step 2^20 ahead of theirs and everything beside one 2^28 ahead; that took 36.2 us for 32 sequences of 2048, this 36.7, and asked
+// of the weights themselves it was 37.8.)
 // The order of the summed axis is free as long as both operands share it: a thread reads 16 or 32 neighbouring codes of a key (q is laid out to
 // match), and 8 or 16 neighbouring codes of four values, whose bytes it exchanges by pairs; no ldmatrix, which cannot split bytes.
 // (Codes to bf16 by two masks and an addition for both products, and a maximum renewed for every tile: 54 us for 32 sequences of 2048, 755 instructions per
 // warp and tile.)
 //
-// Measured (32 query and 8 KV heads of 128): 2 sequences of 65536 positions 57.2 us = 4.84 TB/s, the loops over the tiles 6.3; 32 of 2048 36.5 us (21 at the
+// Measured (32 query and 8 KV heads of 128): 2 sequences of 65536 positions 57.8 us = 4.79 TB/s, the loops over the tiles 6.2; 32 of 2048 36.7 us (21 at the
 // measured copy rate: the ranges are found in 1.3 us, the loops take 27, the joins 4); 1 of 2048 10.9 us.  A tile takes a warp 475 instructions, issued in 44% of
 // the cycles: most of the waiting is for results of the instruction before.  Requests further ahead in L2, queries asked for ahead, and whole units for a CTA
 // without joins were no faster.
@@ -37,7 +41,8 @@ constexpr int A8_STAGES = 3;
 constexpr int A8_SPLITS = 320;    // CTAs that a unit is cut into at most (one more where it begins inside a range)
 constexpr int A8_TICKETS = 1024;  // one per CTA, and one more for the first step of a merge in two
 constexpr int A8_GROUP = 12;      // partial results that are merged in that step
-constexpr float A8_AHEAD = 8.f;   // log2 of how far a score may be ahead of the maximum in use
+constexpr float A8_AHEAD = 8.f;   // log2 of how far a score may be ahead of the largest when the reference was taken
+constexpr float A8_ROOM = 10.f;   // log2 of how far p * v_step may be ahead of the largest when its reference was taken
 constexpr float A8_DIGITS = 127.f * 65536.f;  // the largest number of three digits whose first one is at most 127
 
 __device__ __forceinline__ uint32_t a8_smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -445,7 +450,8 @@ __global__ void __launch_bounds__(A8_THREADS, MT == 1 ? 3 : 2) attn_decode_i8_ke
 
     uint32_t qa[MT][STEPS][6];  // first digits, second digits, third digits of a step's 4 + 4 values
     float o[MT][NT][4], m_run[MT], l_run[MT], q_step[MT];
-    float v_top = 0.f, v_to = 0.f;  // the power of two that value steps are taken relative to; 2^7 over it
+    float s_end[MT], w_to[MT];  // how large a score may get before the references are renewed; 2^15 over how large p * v_step may get
+    float v_end = 0.f;          // how large a value's step may get
     int stage = 0;
     bool fresh = true;
     for (; gt < gt1; ++gt) {
@@ -508,9 +514,9 @@ __global__ void __launch_bounds__(A8_THREADS, MT == 1 ? 3 : 2) attn_decode_i8_ke
                 for (int j = 0; j < NT; ++j) o[m][j][0] = o[m][j][1] = o[m][j][2] = o[m][j][3] = 0.f;
                 m_run[m] = -INFINITY;
                 l_run[m] = 0.f;
+                s_end[m] = -INFINITY;
+                w_to[m] = 1.f;
             }
-            v_top = 7.8886090522101181e-31f;
-            v_to = 128.f / 7.8886090522101181e-31f;
         }
         const int left = what.x & 31;
         if (left > 0) {
@@ -546,25 +552,35 @@ __global__ void __launch_bounds__(A8_THREADS, MT == 1 ? 3 : 2) attn_decode_i8_ke
                     for (int i = 0; i < 4; ++i)
                         if (at[i] >= left) s[m][i] = -INFINITY;
             }
-            // ---- another reference for the scores or for the value steps: rare behind the first tiles
-            float top_v = fmaxf(fmaxf(va.x, va.y), fmaxf(vb.x, vb.y));
-            bool renew = top_v > v_top;
+            // ---- other references for the scores or for p * v_step: rare behind the first tiles
+            const auto largest = [](float x, float y, float z, float w) { return fmaxf(fmaxf(x, y), fmaxf(z, w)); };
+            float top_v = largest(fabsf(va.x), fabsf(va.y), fabsf(vb.x), fabsf(vb.y));
+            bool renew = top_v > v_end;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) renew = renew || fmaxf(fmaxf(s[m][0], s[m][1]), fmaxf(s[m][2], s[m][3])) > m_run[m] + A8_AHEAD;
+            for (int m = 0; m < MT; ++m) renew = renew || largest(s[m][0], s[m][1], s[m][2], s[m][3]) > s_end[m];
             if (__any_sync(0xffffffffu, renew)) {
+                const auto above = [](float v) { return static_cast<float>(static_cast<int>(__float_as_uint(v) >> 23 & 255u) - 126); };  // log2 of a power of two above |v|
+                const float lv[4] = {above(va.x), above(va.y), above(vb.x), above(vb.y)};
                 top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, 1));
                 top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, 2));  // the same positions in all rows
-                const float above = fmaxf(v_top, __uint_as_float((__float_as_uint(top_v) + 0x7fffffu) & 0x7f800000u)), v_corr = v_top / above;
-                v_top = above;
-                v_to = 128.f / above;
+                v_end = __uint_as_float((__float_as_uint(top_v) + 0x7fffffu) & 0x7f800000u);  // of this tile: one that was larger without weight is behind
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    float mx = fmaxf(fmaxf(s[m][0], s[m][1]), fmaxf(s[m][2], s[m][3]));
+                    float mx = largest(s[m][0], s[m][1], s[m][2], s[m][3]), end = static_cast<float>(127 + 15 - static_cast<int>(__float_as_uint(w_to[m]) >> 23));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)), m_run[m]);
-                    const float corr = mx == -INFINITY ? 1.f : a8_exp2(m_run[m] - mx), both = corr * v_corr;
-                    m_run[m] = mx;
-                    l_run[m] *= corr;
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    if (mx > m_run[m]) {  // whole numbers: powers of two exactly
+                        mx = ceilf(mx) + A8_AHEAD;
+                        l_run[m] *= a8_exp2(m_run[m] - mx);
+                        end += m_run[m] - mx;
+                        m_run[m] = mx;
+                    }
+                    float wx = largest(s[m][0] - m_run[m] + lv[0], s[m][1] - m_run[m] + lv[1], s[m][2] - m_run[m] + lv[2], s[m][3] - m_run[m] + lv[3]);
+                    wx = fmaxf(wx, __shfl_xor_sync(0xffffffffu, wx, 1));
+                    wx = fmaxf(wx, __shfl_xor_sync(0xffffffffu, wx, 2));
+                    const float w_end = fmaxf(fmaxf(end, ceilf(wx) + A8_ROOM), -111.f), both = a8_exp2(end - w_end);
+                    w_to[m] = __int_as_float((127 + 15 - static_cast<int>(w_end)) << 23);
+                    s_end[m] = __fadd_rd(m_run[m], fminf(0.f, w_end - above(top_v)));
 #pragma unroll
                     for (int j = 0; j < NT; ++j) { o[m][j][0] *= both; o[m][j][1] *= both; o[m][j][2] *= both; o[m][j][3] *= both; }
                 }
@@ -577,8 +593,8 @@ __global__ void __launch_bounds__(A8_THREADS, MT == 1 ? 3 : 2) attn_decode_i8_ke
 #pragma unroll
                 for (int i = 0; i < 4; ++i) pe[i] = a8_exp2(s[m][i] - base);
                 l_run[m] += (pe[0] + pe[1]) + (pe[2] + pe[3]);  // this thread's positions; the four threads of a row are summed at the end
-                a8_split(pe[0] * (va.x * v_to), pe[1] * (va.y * v_to), pa[m][0], pa[m][1]);
-                a8_split(pe[2] * (vb.x * v_to), pe[3] * (vb.y * v_to), pa[m][2], pa[m][3]);
+                a8_split(pe[0] * va.x * w_to[m], pe[1] * va.y * w_to[m], pa[m][0], pa[m][1]);
+                a8_split(pe[2] * vb.x * w_to[m], pe[3] * vb.y * w_to[m], pa[m][2], pa[m][3]);
             }
             // ---- O += P V: this thread's D / 8 neighbouring codes (from g * D / 8 on) of positions 2 t4, + 1, + 8, + 9
             uint32_t w[4][NT / 4];
@@ -614,16 +630,16 @@ __global__ void __launch_bounds__(A8_THREADS, MT == 1 ? 3 : 2) attn_decode_i8_ke
         // ---- this CTA's share of the unit is complete: merge the warps, each of which saw a quarter of every tile's positions
         const int kvh = what.w / p.blocks, h0 = (what.w - kvh * p.blocks) * ROWS, rows = min(ROWS, p.G - h0);
         const int64_t out0 = static_cast<int64_t>(what.z) * p.nq * D + (static_cast<int64_t>(kvh) * p.G + h0) * D;
-        const float v_of = v_top * (1.f / 128.f);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
+            const float w_of = __uint_as_float(0x7f000000u - __float_as_uint(w_to[m]));  // 1 over a power of two
             float l = l_run[m];
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if (t4 == 0) *reinterpret_cast<float2*>(red_ml + (warp * ROWS + m * 8 + g) * 2) = make_float2(m_run[m], l);
 #pragma unroll
             for (int j = 0; j < NT; ++j)  // column 2 t4 + e of instruction j is value (2 t4 + e) * NT + j of the head: kept at 8 j + 2 t4 + e
-                *reinterpret_cast<float2*>(red_o + (warp * ROWS + m * 8 + g) * RED + 8 * j + 2 * t4) = make_float2((o[m][j][0] + o[m][j][2]) * v_of, (o[m][j][1] + o[m][j][3]) * v_of);
+                *reinterpret_cast<float2*>(red_o + (warp * ROWS + m * 8 + g) * RED + 8 * j + 2 * t4) = make_float2((o[m][j][0] + o[m][j][2]) * w_of, (o[m][j][1] + o[m][j][3]) * w_of);
         }
         __syncthreads();
         const int plan_r = s_plan[0], tiles = what.x >> 5, unit_start = gt - (what.y >> 1);  // the number of the unit's first tile
