@@ -424,14 +424,30 @@ std::pair<const int64_t*, int> positions(const at::Tensor* pos, int64_t B, const
         raise(PyExc_ValueError, message(name, " needs int64 positions: a scalar, or one for each of the ", B, " sequences with unit stride; got ", pos->scalar_type(), " ", pos->sizes()));
     return {static_cast<const int64_t*>(pos->data_ptr()), one ? 0 : 1};
 }
+// Elements of each of the `rows` rows that t is: of shape [rows, width], or contiguous with the rows in its leading dimensions (one at least, unless t is a single
+// row) and behind them a width, heads of D, groups of heads for each of nkv, each with ones wherever.  A number of rows that is another one is never taken for heads.
+int64_t row_width(const at::Tensor& t, int64_t rows, int64_t nkv, int64_t D, const char* name) {
+    const auto dims = t.sizes();
+    if (dims.size() == 2) {
+        if (dims[0] == rows) return dims[1];
+    } else if (t.is_contiguous() && !dims.empty()) {
+        size_t i = 0;
+        int64_t front = 1;
+        if (dims.size() > 2 || rows != 1)
+            for (front = dims[i++]; front != rows && i < dims.size(); ++i) front *= dims[i];
+        std::vector<int64_t> rest;
+        for (; i < dims.size(); ++i)
+            if (dims[i] != 1) rest.push_back(dims[i]);
+        const bool heads = rest.size() <= 1 || (rest.size() == 2 && (rest[1] == D || rest[0] == nkv)) || (rest.size() == 3 && rest[0] == nkv && rest[2] == D);
+        if (front == rows && heads) return t.numel() / rows;
+    }
+    raise(PyExc_ValueError, message(name, " must have ", rows, " row(s), as the cache and the number of new tokens say, two-dimensional or contiguous; got ", t.sizes(), " with strides ", t.strides()));
+}
 // elements from one row of `width` to the next: contiguous in any shape, or two-dimensional with unit inner stride
-int64_t row_stride(const at::Tensor& t, int64_t rows, int64_t width, const char* name, at::ScalarType type) {
-    if (t.scalar_type() == type) {
-        if (t.is_contiguous()) {
-            if (t.numel() >= rows * width) return width;
-        } else if (t.dim() == 2 && t.size(0) >= rows && t.size(1) == width && t.stride(1) == 1 && (t.stride(0) >= width || rows == 1)) {
-            return std::max(t.stride(0), width);
-        }
+int64_t row_stride(const at::Tensor& t, int64_t rows, int64_t width, int64_t nkv, int64_t D, const char* name, at::ScalarType type) {
+    if (t.scalar_type() == type && row_width(t, rows, nkv, D, name) == width) {
+        if (t.is_contiguous()) return width;
+        if (t.dim() == 2 && t.stride(1) == 1 && (t.stride(0) >= width || rows == 1)) return std::max(t.stride(0), width);
     }
     raise(PyExc_ValueError, message(name, " must be ", type, " rows [", rows, ", ", width, "], contiguous or two-dimensional with unit inner stride; got ", t.scalar_type(), " ", t.sizes(),
                                      " with strides ", t.strides()));
@@ -447,14 +463,14 @@ PyObject* rope_kv_i8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const CacheI8 c = cache_i8(a[6], "rope_kv_i8_", {&q, &k, &v, &cos, &sin, &pos, given});
         const int64_t s = long_arg(a[7]);
         const at::Tensor& out = given ? *given : q;
-        if (s < 0 || !half_type(q.scalar_type())) raise(PyExc_ValueError, message("rope_kv_i8_ needs bf16 or f16 tensors and s >= 0, got ", q.scalar_type(), " and ", s));
+        if (s < 0 || s > INT32_MAX || !half_type(q.scalar_type())) raise(PyExc_ValueError, message("rope_kv_i8_ needs bf16 or f16 tensors and s of 0 to 2^31 - 1, got ", q.scalar_type(), " and ", s));
         if (c.B && s) {
-            const int64_t rows = c.B * s, heads = rows * c.D > 0 ? q.numel() / (rows * c.D) : 0;
+            const int64_t rows = c.B * s, heads = row_width(q, rows, c.nkv, c.D, "q") / std::max<int64_t>(c.D, 1);
             for (const at::Tensor* t : {&cos, &sin})
-                if (t->scalar_type() != at::kFloat || t->numel() < c.T * (c.D / 2) || !t->is_contiguous())
-                    raise(PyExc_ValueError, "rope_kv_i8_ needs contiguous float32 rotary tables of T rows");
-            const int64_t ldq = row_stride(q, rows, heads * c.D, "q", q.scalar_type()), ldo = row_stride(out, rows, heads * c.D, "out", q.scalar_type());
-            const int64_t ldk = row_stride(k, rows, c.nkv * c.D, "k", q.scalar_type()), ldv = row_stride(v, rows, c.nkv * c.D, "v", q.scalar_type());
+                if (t->scalar_type() != at::kFloat || t->dim() < 2 || t->size(-1) != c.D / 2 || t->numel() < c.T * (c.D / 2) || !t->is_contiguous())
+                    raise(PyExc_ValueError, message("rope_kv_i8_ needs contiguous float32 rotary tables [T, D/2] = [", c.T, ", ", c.D / 2, "] or longer; got ", t->scalar_type(), " ", t->sizes()));
+            const auto stride = [&](const at::Tensor& t, int64_t n, const char* name) { return row_stride(t, rows, n * c.D, c.nkv, c.D, name, q.scalar_type()); };
+            const int64_t ldq = stride(q, heads, "q"), ldo = stride(out, heads, "out"), ldk = stride(k, c.nkv, "k"), ldv = stride(v, c.nkv, "v");
             if (ldk != ldv) raise(PyExc_ValueError, message("k and v must have the same row stride, got ", ldk, " and ", ldv));
             const auto at = positions(&pos, c.B, "rope_kv_i8_");
             const unsigned flags = pdl_flag(a[9]);
@@ -528,9 +544,9 @@ PyObject* attn_decode_i8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const at::Tensor& q = tensor(a[0]);
         const at::Tensor *pos = optional_tensor(a[2]), *given = optional_tensor(a[3]), *workspace = optional_tensor(a[6]);
         const CacheI8 c = cache_i8(a[1], "attn_decode_i8", {&q, pos, given, workspace});
-        if (!half_type(q.scalar_type()) || q.dim() < 1 || c.D < 1 || (c.B && q.numel() % (c.B * c.D)))
+        if (!half_type(q.scalar_type()) || q.dim() < 1 || c.D < 1)
             raise(PyExc_ValueError, message("attn_decode_i8 needs bf16 or f16 queries [B, nq*D], got ", q.scalar_type(), " ", q.sizes()));
-        const int64_t nq = c.B ? q.numel() / (c.B * c.D) : q.size(-1) / c.D;
+        const int64_t nq = (c.B ? row_width(q, c.B, c.nkv, c.D, "q") : q.size(-1)) / c.D;
         if (given && (given->scalar_type() != q.scalar_type() || given->numel() != q.numel() || !given->is_contiguous()))
             raise(PyExc_ValueError, "attn_decode_i8 needs a contiguous output of the type and size of q");
         if (workspace && (workspace->element_size() != 1 || !workspace->is_contiguous())) raise(PyExc_ValueError, "attn_decode_i8 needs a workspace of contiguous bytes");
@@ -540,7 +556,7 @@ PyObject* attn_decode_i8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const at::Tensor out = given ? *given : at::empty({c.B, nq * c.D}, q.options());
         if (c.B) {
             const auto at = positions(pos, c.B, "attn_decode_i8");
-            const int64_t ldq = row_stride(q, c.B, nq * c.D, "q", q.scalar_type());
+            const int64_t ldq = row_stride(q, c.B, nq * c.D, c.nkv, c.D, "q", q.scalar_type());
             const auto from = reinterpret_cast<uintptr_t>(q.data_ptr()), to = reinterpret_cast<uintptr_t>(out.data_ptr());
             if (to < from + 2 * ((c.B - 1) * ldq + nq * c.D) && from < to + 2 * c.B * nq * c.D)
                 raise(PyExc_ValueError, "attn_decode_i8 cannot write over q: parts of a sequence that run later still read it");

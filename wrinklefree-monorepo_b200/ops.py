@@ -630,8 +630,8 @@ def kv_cache_i8(b: int, nkv: int, t: int, d: int, device) -> KVCacheI8:
 def rope_kv_i8_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, cache: KVCacheI8, s: int = 1,
                 out: Optional[torch.Tensor] = None, pdl: bool = True) -> torch.Tensor:
     """RoPE of `s` new tokens per sequence and the write of their keys and values into an 8-bit cache, where they are quantized: `rope_kv_`
-    and `rope_kv_prompt_` for a `KVCacheI8`.  q [B*s, nq*D], k, v [B*s, nkv*D], bf16 or f16, contiguous or rows of wider tensors (k and v then equally far
-    apart); cos, sin float32 [T, D/2].  `pos`: int64 scalar on the device, or one per sequence [B], the position of a sequence's first new token; a
+    and `rope_kv_prompt_` for a `KVCacheI8`.  q [B*s, nq*D], k, v [B*s, nkv*D], bf16 or f16, contiguous (tokens and heads in dimensions of
+    their own if wanted) or rows of wider tensors (k and v then equally far apart), as many as the cache and `s` say; cos, sin float32 [T, D/2].  `pos`: int64 scalar on the device, or one per sequence [B], the position of a sequence's first new token; a
     token whose position is not in the cache (a slot without a sequence has a negative one) is not written, and its query becomes zero.  The
     rotated queries go to `out` [B*s, nq*D] (default: in place) and are returned.  `pdl`: the launch may start while its predecessor in the stream ends; it touches
     nothing before that has ended, so this is the default here and in the other operators on 8-bit caches."""
@@ -652,7 +652,7 @@ def attn_i8_workspace(nq: int, nkv: int, d: int, device) -> torch.Tensor:
 
 def attn_decode_i8(q: torch.Tensor, cache: KVCacheI8, pos: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                    pdl: bool = True, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Decode-step attention over an 8-bit cache: `attn_decode` for a `KVCacheI8`.  q [B, nq*D] (rotated; bf16 or f16, rows may be wider apart), `pos` an int64
+    """Decode-step attention over an 8-bit cache: `attn_decode` for a `KVCacheI8`.  q [B, nq*D] (rotated; bf16 or f16, rows may be wider apart; contiguous also [B, nq, D]), `pos` an int64
     scalar on the device or one per sequence [B]: sequence b attends to its positions 0 .. pos[b], to none where that is negative (its output is zero); None: to all
     T.  Any number of query heads per KV head.  Returns out [B, nq*D] of q's type.  `workspace`: from `attn_i8_workspace`, kept by the caller (a captured
     call without one clears its own on every replay)."""
