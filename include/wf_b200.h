@@ -441,7 +441,7 @@ int wf_argmax_bf16(const void* x, int64_t ld, int64_t B, int64_t V, int64_t* out
  *
  * An int8 KV cache holds codes [B, nkv, T, D] and steps [B, nkv, T] of its keys and of its values, one row per head and position.
  * wf_rope_kv_i8: S new tokens per sequence, token s of sequence b at position p = pos[b * pos_stride] + s (pos_stride 0 or 1): q_out = q rotated by p
- * (q_out may be q), k rotated and quantized, v quantized, both written at p.  q, q_out: rows b * S + s of nq * D, strides ldq, ldo; k, v:
+ * (q_out may be q, but else shares nothing with q, k or v), k rotated and quantized, v quantized, both written at p.  q, q_out: rows b * S + s of nq * D, strides ldq, ldo; k, v:
  * rows of nkv * D, stride ldkv; bf16 or f16, strides multiples of 8.  cos, sin: [T, D/2].  A position outside 0 .. T - 1 writes nothing, and its row of
  * q_out is zero.  wf_kv_read_i8: positions start .. start + S - 1 as bf16 or f16, k and v [units, S, D], units = B * nkv.  D = 64 or 128; tensors 16-byte aligned (the steps
  * 4-byte).  The quantized form of wf_rope_kv_bf16 (apply_rotary_emb, packages/training/src/wrinklefree/models/attention.py:41-64; the cache of
@@ -457,7 +457,7 @@ int wf_kv_read_i8(const int8_t* kcache, const int8_t* vcache, const float* kscal
 /*
  * wf_attn_decode_bf16 over an int8 cache: q [B, nq * D] (row stride ldq, bf16 or f16, rotated), out [B, nq * D] of the same type.  Sequence b attends to
  * the positions 0 .. pos[b * pos_stride] (pos null: all T; below 0: none, its row of out is zero).  nq a multiple of nkv; D = 64 or 128.
- * Nothing beyond a sequence's positions is read.  workspace: wf_attn_decode_i8_workspace_bytes(...) bytes, 256-byte aligned, ZERO before its first use
+ * Nothing beyond a sequence's positions is read.  out must not overlap q.  workspace: wf_attn_decode_i8_workspace_bytes(...) bytes, 256-byte aligned, ZERO before its first use
  * (every launch leaves it so that the next finds its tickets zero); launches that run one after another may share it, in any shapes that need no more.
  * Takes WF_FLAG_PDL.
  */

@@ -58,3 +58,23 @@ def test_other_numbers_of_rows_are_not_taken_for_heads(wf):
         with pytest.raises(ValueError):
             bad()
     assert all(torch.equal(a, b) for a, b in zip(cache, before))
+
+
+def test_outputs_beside_the_inputs(wf):
+    """Rotated queries between the columns of one tensor with q, k and v; an output that shares rows with them in any other way is refused."""
+    q, k, v, cos, sin, pos, cache = setup(wf, S)
+    two = copies(cache)
+    want = wf.ops.rope_kv_i8_(q, k, v, cos, sin, pos, cache, S, out=torch.empty_like(q))
+    n, m = NQ * D, NKV * D
+    room = torch.zeros(B * S + 1, 2 * (n + m) + 8, dtype=torch.bfloat16, device=DEV)
+    cols = [room[:B * S, a:a + w] for a, w in ((0, n), (n, m), (n + m, m), (n + 2 * m, n))]
+    for c, x in zip(cols, (q, k, v)):
+        c.copy_(x)
+    assert torch.equal(wf.ops.rope_kv_i8_(*cols[:3], cos, sin, pos, two, S, out=cols[3]), want) and torch.equal(cols[0], q)
+    assert all(torch.equal(a, b) for a, b in zip(cache, two))
+    flat = torch.zeros(4 * B * S * n, dtype=torch.bfloat16, device=DEV)
+    for q2, out in ((cols[0], room[1:, :n]), (cols[0], room[:B * S, 8:8 + n]), (cols[3], room[:B * S, n:2 * n]), (flat[:q.numel()].view_as(q), flat[D:D + q.numel()].view_as(q))):
+        with pytest.raises(RuntimeError, match="share"):
+            wf.ops.rope_kv_i8_(q2, *cols[1:3], cos, sin, pos, two, S, out=out)
+    got = wf.ops.rope_kv_i8_(flat[:q.numel()].view_as(q).copy_(q), k, v, cos, sin, pos, two, S, out=flat[q.numel():2 * q.numel()].view_as(q))  # one behind the other
+    assert torch.equal(got, want)

@@ -746,6 +746,9 @@ extern "C" int wf_attn_decode_i8(const void* q, int dtype, int64_t ldq, const in
     const size_t need = wf_attn_decode_i8_workspace_bytes(nq, nkv, D);
     if (!workspace || workspace_bytes < need) return fail(WF_E_SCRATCH, "wf_attn_decode_i8: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0, need);
     WF_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "wf_attn_decode_i8: workspace must be 256-byte aligned");
+    const auto from = reinterpret_cast<uintptr_t>(q), to = reinterpret_cast<uintptr_t>(out);
+    WF_REQUIRE(to >= from + 2 * ((B - 1) * ldq + static_cast<int64_t>(nq) * D) || from >= to + 2 * B * nq * D,
+               "wf_attn_decode_i8: out must not overlap q, which parts of a sequence that run later still read");
     if (int rc = require_device()) return rc;
     AttnI8Params p;
     p.q = q; p.k = kcache; p.v = vcache; p.ks = kscale; p.vs = vscale; p.pos = pos; p.out = out;

@@ -359,6 +359,19 @@ static bool aligned16(std::initializer_list<const void*> ps) {
         if (reinterpret_cast<uintptr_t>(q) & 15) return false;
     return true;
 }
+// Whether one of `rows` rows of a (wa bytes each, lda apart) shares a byte with one of as many of b.  Rows equally far apart may lie between each other, like columns of
+// one tensor; of others whose ranges meet it is taken to be so.
+static bool rows_meet(const void* a, int64_t wa, int64_t lda, const void* b, int64_t wb, int64_t ldb, int64_t rows) {
+    const int64_t from_a_to_b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(a));
+    if (from_a_to_b >= (rows - 1) * lda + wa || -from_a_to_b >= (rows - 1) * ldb + wb) return false;
+    if (rows == 1 || lda != ldb) return true;
+    // the first row of b, counted from one of a's, that ends behind that one's beginning
+    int64_t first = (-wb - from_a_to_b) / lda;
+    while (from_a_to_b + first * lda + wb <= 0) ++first;
+    while (first > -(rows - 1) && from_a_to_b + (first - 1) * lda + wb > 0) --first;
+    if (first < -(rows - 1)) first = -(rows - 1);
+    return first < rows && from_a_to_b + first * lda < wa;
+}
 
 }  // namespace wf
 
@@ -376,6 +389,11 @@ extern "C" int wf_rope_kv_i8(const void* q, int64_t ldq, const void* k, const vo
                "wf_rope_kv_i8: row strides must cover the heads and be multiples of 8");
     WF_REQUIRE(aligned16({q, k, v, cos, sin, q_out, kcache, vcache}), "wf_rope_kv_i8: tensors must be 16-byte aligned");
     WF_REQUIRE(B * S < (1LL << 31), "wf_rope_kv_i8: oversized problem");
+    const int64_t wq = 2LL * nq * D, wk = 2LL * nkv * D, rows_all = B * S;
+    const bool in_place = q_out == q && (ldo == ldq || rows_all == 1);
+    WF_REQUIRE((in_place || !rows_meet(q_out, wq, 2 * ldo, q, wq, 2 * ldq, rows_all)) && !rows_meet(q_out, wq, 2 * ldo, k, wk, 2 * ldkv, rows_all) &&
+                   !rows_meet(q_out, wq, 2 * ldo, v, wk, 2 * ldkv, rows_all),
+               "wf_rope_kv_i8: q_out must be q itself or share nothing with q, k and v, which other threads still read");
     if (int rc = require_device()) return rc;
     RopeI8Params p;
     p.q = q; p.k = k; p.v = v; p.q_out = q_out; p.cos = cos; p.sin = sin; p.pos = pos;

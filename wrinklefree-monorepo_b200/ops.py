@@ -633,7 +633,7 @@ def rope_kv_i8_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     and `rope_kv_prompt_` for a `KVCacheI8`.  q [B*s, nq*D], k, v [B*s, nkv*D], bf16 or f16, contiguous (tokens and heads in dimensions of
     their own if wanted) or rows of wider tensors (k and v then equally far apart), as many as the cache and `s` say; cos, sin float32 [T, D/2].  `pos`: int64 scalar on the device, or one per sequence [B], the position of a sequence's first new token; a
     token whose position is not in the cache (a slot without a sequence has a negative one) is not written, and its query becomes zero.  The
-    rotated queries go to `out` [B*s, nq*D] (default: in place) and are returned.  `pdl`: the launch may start while its predecessor in the stream ends; it touches
+    rotated queries go to `out` [B*s, nq*D] (default: in place; another one may lie between the columns of q, k and v but share nothing with them) and are returned.  `pdl`: the launch may start while its predecessor in the stream ends; it touches
     nothing before that has ended, so this is the default here and in the other operators on 8-bit caches."""
     return L.host().rope_kv_i8(q, k, v, cos, sin, pos, cache, s, out, pdl)
 
