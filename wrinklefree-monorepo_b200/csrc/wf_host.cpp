@@ -666,6 +666,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             raise(PyExc_ValueError, message("token_logprobs needs logits [..., V] of float32, bf16 or f16, got ", logits.scalar_type(), " ", logits.sizes()));
         if (given.scalar_type() != at::kLong || given.sizes() != logits.sizes().slice(0, logits.dim() - 1) || given.device() != logits.device())
             raise(PyExc_ValueError, message("token_logprobs needs int64 tokens ", logits.sizes().slice(0, logits.dim() - 1), " on the logits' device, got ", given.scalar_type(), " ", given.sizes()));
+        if (logits._fw_grad(0).defined()) raise(PyExc_NotImplementedError, "token_logprobs has no forward-mode derivative");
         if (top < 0 || top > 32) raise(PyExc_ValueError, message("token_logprobs finds 0 to 32 alternatives, asked for ", top));
         c10::cuda::CUDAGuard guard(logits.device());
         const int64_t v = logits.size(-1);

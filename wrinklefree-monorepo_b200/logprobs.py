@@ -51,7 +51,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     of -inf are masked: they have no probability and are never an alternative (index -1 and -inf where fewer than `top` are left); a row of nothing
     else has a log probability of -inf and an entropy of 0, and no gradient.  A row that holds a NaN or +inf gives NaN; a NaN is never an alternative.
 
-    Differentiable (once) in the logits through the log probabilities, the entropy and the alternatives' log probabilities.  As for any operator, a backward
+    Differentiable (once, in reverse mode; logits with a tangent are refused) in the logits through the log probabilities, the entropy and the alternatives' log probabilities.  As for any operator, a backward
     pass is captured into a CUDA graph only while no eager autograd graph of the same leaves is alive."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top))

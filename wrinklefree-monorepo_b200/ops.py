@@ -655,7 +655,7 @@ def attn_decode_i8(q: torch.Tensor, cache: KVCacheI8, pos: Optional[torch.Tensor
     """Decode-step attention over an 8-bit cache: `attn_decode` for a `KVCacheI8`.  q [B, nq*D] (rotated; bf16 or f16, rows may be wider apart; contiguous also [B, nq, D]), `pos` an int64
     scalar on the device or one per sequence [B]: sequence b attends to its positions 0 .. pos[b], to none where that is negative (its output is zero); None: to all
     T.  Any number of query heads per KV head.  Returns out [B, nq*D] of q's type.  `workspace`: from `attn_i8_workspace`, kept by the caller (a captured
-    call without one clears its own on every replay)."""
+    call without one clears its own on every replay).  For serving, as all operators on 8-bit caches: no gradients."""
     return L.host().attn_decode_i8(q, cache, pos, out, scale, pdl, workspace)
 
 
@@ -738,7 +738,8 @@ def linear_i8(x: torch.Tensor, codes: torch.Tensor, w_scale: torch.Tensor, x_sca
     float type, quantized per token by the same rule on the way, or int8 codes with x_scale [tokens] (rows 16-byte aligned and a multiple of
     16 bytes apart).  The sums are exact; y = (float(sum) * x_scale) * w_scale + bias, rounded once more to `out_dtype` (default: x's type,
     bf16 for int8 tokens).  `out`: [..., N] with unit inner stride.  K up to 131071.  `pdl`, for int8 tokens: the launch may start while its predecessors in
-    the stream end; those may write the tokens and their scales, not the weights' codes and scales."""
+    the stream end; those may write the tokens and their scales, not the weights' codes and scales.  For serving: the result has no graph and no tangent, also
+    where x or the bias require gradients."""
     return L.host().linear_i8(x, codes, w_scale, x_scale, bias, out, out_dtype, pdl)
 
 
