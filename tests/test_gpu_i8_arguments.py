@@ -78,3 +78,28 @@ def test_outputs_beside_the_inputs(wf):
             wf.ops.rope_kv_i8_(q2, *cols[1:3], cos, sin, pos, two, S, out=out)
     got = wf.ops.rope_kv_i8_(flat[:q.numel()].view_as(q).copy_(q), k, v, cos, sin, pos, two, S, out=flat[q.numel():2 * q.numel()].view_as(q))  # one behind the other
     assert torch.equal(got, want)
+
+
+def test_workspaces_of_streams_that_are_not_torchs_own(wf):
+    """Nothing is kept for them beyond the call: their handles do not say which stream it is."""
+    q, k, v, cos, sin, pos, cache = setup(wf, 1)
+    want, own = wf.ops.attn_decode_i8(q, cache, pos), torch.cuda.Stream()
+    foreign = torch.cuda.ExternalStream(torch.cuda.Stream().cuda_stream)
+    torch.cuda.synchronize()
+
+    def kept(stream):
+        before = torch.cuda.memory_allocated()
+        with torch.cuda.stream(stream):
+            for _ in range(3):
+                got = wf.ops.attn_decode_i8(q, cache, pos)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del got
+        return torch.cuda.memory_allocated() - before
+
+    kept(own)
+    assert kept(own) == 0  # the one that is kept
+    assert kept(foreign) == 0
+    with torch.cuda.stream(torch.cuda.ExternalStream(2)):  # the per-thread default stream
+        with pytest.raises(ValueError, match="workspace"):
+            wf.ops.attn_decode_i8(q, cache, pos)

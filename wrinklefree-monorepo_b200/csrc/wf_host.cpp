@@ -513,17 +513,22 @@ PyObject* kv_read_i8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 // Workspaces of attn_decode_i8 calls that bring none, by device and stream: launches of one stream run one after the other, and the memory goes back to
-// that stream.  A captured call gets one of the graph's own, cleared on every replay.  (Never destroyed: the process's end does not wait for this library.)
+// that stream.  A captured call gets one of the graph's own, cleared on every replay.  A stream that is not torch's own (its id is its handle) gets one for the
+// call: when such a stream is destroyed another may have its handle.  The per-thread default stream has one handle for a stream in every thread, which the
+// allocator does not know either: there the workspace is the caller's.  (Never destroyed: the process's end does not wait for this library.)
 constexpr size_t KEPT_WORKSPACES = 16;
 struct KeptWorkspace {
     int device;
     void* stream;
     at::Tensor ws;
 };
-at::Tensor stream_workspace(int64_t bytes, const at::Tensor& like, void* stream) {
+at::Tensor stream_workspace(int64_t bytes, const at::Tensor& like, const c10::cuda::CUDAStream& current) {
     static std::vector<KeptWorkspace>& kept = *new std::vector<KeptWorkspace>();
     const auto options = like.options().dtype(at::kByte);
+    void* const stream = current.stream();
+    if (stream == cudaStreamPerThread) raise(PyExc_ValueError, "attn_decode_i8 needs a workspace of the caller's on the per-thread default stream");
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return at::zeros({bytes}, options);
+    if (stream && current.id() == static_cast<c10::StreamId>(reinterpret_cast<intptr_t>(stream))) return at::zeros({bytes}, options);
     const int device = like.device().index();
     for (size_t i = 0; i < kept.size(); ++i)
         if (kept[i].device == device && kept[i].stream == stream) {
@@ -560,12 +565,12 @@ PyObject* attn_decode_i8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             const auto from = reinterpret_cast<uintptr_t>(q.data_ptr()), to = reinterpret_cast<uintptr_t>(out.data_ptr());
             if (to < from + 2 * ((c.B - 1) * ldq + nq * c.D) && from < to + 2 * c.B * nq * c.D)
                 raise(PyExc_ValueError, "attn_decode_i8 cannot write over q: parts of a sequence that run later still read it");
-            void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+            const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream();
             const at::Tensor ws = workspace ? *workspace
-                                            : stream_workspace(static_cast<int64_t>(std::max<size_t>(wf_attn_decode_i8_workspace_bytes(static_cast<int>(nq), static_cast<int>(c.nkv), static_cast<int>(c.D)), 1)), q, stream);
+                                            : stream_workspace(static_cast<int64_t>(std::max<size_t>(wf_attn_decode_i8_workspace_bytes(static_cast<int>(nq), static_cast<int>(c.nkv), static_cast<int>(c.D)), 1)), q, current);
             check(wf_attn_decode_i8(q.data_ptr(), dtype_code(q.scalar_type()), ldq, c.kp(), c.vp(), c.ksp(), c.vsp(), at.first, at.second, out.data_ptr(), c.B,
                                     static_cast<int>(nq), static_cast<int>(c.nkv), static_cast<int>(c.D), c.T, static_cast<float>(scale), ws.data_ptr(),
-                                    static_cast<size_t>(ws.numel()), flags, stream),
+                                    static_cast<size_t>(ws.numel()), flags, current.stream()),
                   "wf_attn_decode_i8");
         }
         return wrap(out);

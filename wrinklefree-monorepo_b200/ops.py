@@ -655,7 +655,7 @@ def attn_decode_i8(q: torch.Tensor, cache: KVCacheI8, pos: Optional[torch.Tensor
     """Decode-step attention over an 8-bit cache: `attn_decode` for a `KVCacheI8`.  q [B, nq*D] (rotated; bf16 or f16, rows may be wider apart; contiguous also [B, nq, D]), `pos` an int64
     scalar on the device or one per sequence [B]: sequence b attends to its positions 0 .. pos[b], to none where that is negative (its output is zero); None: to all
     T.  Any number of query heads per KV head.  Returns out [B, nq*D] of q's type.  `workspace`: from `attn_i8_workspace`, kept by the caller (a captured
-    call without one clears its own on every replay).  For serving, as all operators on 8-bit caches: no gradients."""
+    call without one clears its own on every replay, one on a stream that is not torch's own every time; the per-thread default stream needs one).  For serving, as all operators on 8-bit caches: no gradients."""
     return L.host().attn_decode_i8(q, cache, pos, out, scale, pdl, workspace)
 
 
