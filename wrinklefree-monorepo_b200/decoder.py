@@ -652,6 +652,9 @@ class TernaryDecoder:
     def score(self, ids: torch.Tensor, top: int = 0) -> TokenLogprobs:
         """What the model makes of given tokens ids [B, S]: the log probability of each token but the first, given those in front of it, the entropy at
         its place and the `top` alternatives (`token_logprobs`), each [B, S - 1].  Fills the cache as `prefill` does."""
+        if not 0 <= top <= TOP_MAX:  # before the cache is filled
+            raise ValueError(f"score finds 0 to {TOP_MAX} alternatives, asked for {top}")
+        ids = ids.to(self.dev, torch.long)  # where the logits will be
         logits = self.prefill(ids, all_logits=True)
         last = torch.full_like(ids[:, :1], -1)  # nothing follows the last one: the logits stay one piece
         return TokenLogprobs(*(t[:, :-1] for t in token_logprobs(logits, torch.cat([ids[:, 1:], last], 1), top)))
