@@ -73,3 +73,19 @@ def test_gradient_of_large_logits(wf, dt, v):
     logp = torch.log_softmax(x.detach().double().cpu(), -1).clamp(min=-200)
     off = 2.0 ** -21 * (4 + logp.abs()) + 2.0 ** -23 * (v / 256 + 64)
     assert ((dx.double().cpu() - want).abs() <= HALF[dt] * want.abs() + off * size + TINY[dt] + 1e-37).all()
+
+
+@pytest.mark.parametrize("n,v", [(3000, 1), (3000, 5), (2000, 1000), (600, 9000), (20, 60000)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+def test_a_row_that_one_token_has_all_of(wf, dt, n, v):
+    """No probability above 1 and no entropy below 0, not even by a rounding: what is taken of them (the logarithm of the rest, a root) would be NaN."""
+    g = torch.Generator(device=DEV).manual_seed(v)
+    x = torch.randn(n, v, generator=g, device=DEV)
+    x[:, v // 2] = torch.exp(torch.rand(n, generator=g, device=DEV) * 7 + 3) + 20
+    x[::2] -= 500
+    x = x.to(dt)
+    tok = torch.full((n,), v // 2, device=DEV)
+    got = wf.token_logprobs(x, tok, top=1)
+    assert (got.logprob <= 0).all() and (got.top_logprob <= 0).all() and (got.entropy >= 0).all() and torch.log1p(-got.logprob.exp()).isnan().sum() == 0
+    for a, w, t in zip(got, *oracle(x, tok, 1)):
+        agree(a, w, t)

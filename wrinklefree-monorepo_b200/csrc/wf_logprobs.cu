@@ -471,13 +471,14 @@ __global__ void __launch_bounds__(LP_THREADS, 7) logprobs_kernel(const LpParams 
         const bool empty = a.s == 0.f;  // every element is -inf
         const float log2_s = log2f(a.s);
         row_m = a.m;
-        row_log = LP_LN2 * (log2_s - lp_rest<DT>(a.m));
+        // neither is below 0 but by rounding, as where one element has all of the row: a logarithm of more than 1 or an entropy of less than nothing is no answer
+        row_log = empty ? -INFINITY : lp_max_nan(LP_LN2 * (log2_s - lp_rest<DT>(a.m)), 0.f);
         if (lane == 0) {
             float lp = 0.f;
             if (tok >= p.V) lp = __uint_as_float(0x7fc00000u);
             else if (tok >= 0) lp = empty ? -INFINITY : (tok_logit - row_m) - row_log;
             p.logprob[row] = lp;
-            p.entropy[row] = empty ? 0.f : LP_LN2 * (log2_s - a.t / a.s);
+            p.entropy[row] = empty ? 0.f : lp_max_nan(LP_LN2 * (log2_s - a.t / a.s), 0.f);
             if (p.stats) {
                 p.stats[2 * row] = row_m;
                 p.stats[2 * row + 1] = row_log;
