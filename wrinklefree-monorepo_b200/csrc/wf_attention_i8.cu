@@ -2,7 +2,7 @@
 //
 //   s[t] = scale * (q . k_codes[t]) * k_step[t]        out = softmax_t(s) @ (v_codes[t] * v_step[t])        t <= pos[b]
 //
-// Every code and step of the context is read once per launch, half the bytes of a bf16 cache: HBM bounds it, as long as the SM's instructions keep
+// Every code and step of the context is read once per launch and sixteen query heads of a KV head, half the bytes of a bf16 cache: HBM bounds it, as long as the SM's instructions keep
 // up: 730 cycles for the 16.9 KB of 64 positions at the measured rate.  The steps never touch the codes: k_step multiplies a score, v_step a probability.
 //
 // Scores: q as three signed 8-bit digits of 2^23 steps of its row's maximum, so that the codes of the keys go into mma.sync.m16n8k32 as they lie in memory

@@ -113,7 +113,9 @@ class TernaryDecoder:
         `fuse_exchange` (tensor parallel, up to 8 sequences, bf16): the row-parallel projections push their partial outputs to every rank inside their own launch and the residual add + RMSNorm that follows sums them (default: from two
         sequences on; True / False force it).
         `cache_dtype` torch.int8 keeps keys and values in 8 bits with a scale per head and position (`ops.KVCacheI8`; layers then run as separate
-        launches, and a prompt attends to what the cache holds, so that a prompt and the same tokens one by one see the same keys); `head_dtype`
+        launches, and a prompt attends to what the cache holds, so that a prompt and the same tokens one by one see the same keys).  It pays where the cache is much of what a step reads: a
+        step of SMOLLM2_135M takes 1049 us for 1388 at 32768 positions, as long at 8192, but 800 for 418 at 256, where the bf16 cache has all layers in one launch; 32 sequences of it 2455 for 2614
+        at 8192, 1827 for 1789 at 2048.  `head_dtype`
         torch.int8 keeps the output head in 8 bits with a scale per vocabulary row.  Both default to `dtype`; a bf16 model can have either."""
         for name, given in (("cache_dtype", cache_dtype), ("head_dtype", head_dtype)):
             if given not in (None, dtype) and (given != torch.int8 or dtype != torch.bfloat16):
